@@ -354,8 +354,10 @@ def grouped_gemm_w4(a, q: W4Experts, tile_expert, out, max_mtiles: int, epilogue
             if tl and at.few_rows(e, at.k, min(rows_in_use, rows)):
                 check(at.few_tiles(at.weight, *ap, *yp, te, tl, max_mtiles, epilogue, at.status, at.sms, stream_ptr()), "grouped_gemm_w4")
                 return out
-            # scratch: the rows in fp16, their factors in 32 bits, the list of items
-            p = a.new_empty(rows * at.pitch + 2 * rows + 8 + 64 * max_mtiles).data_ptr()
+            # the rows in fp16, their factors in 32 bits, the list of items; held until both launches are made: the call lets other threads
+            # run, which may be given what is free
+            scratch = a.new_empty(rows * at.pitch + 2 * rows + 8 + 64 * max_mtiles)
+            p = scratch.data_ptr()
             back = p + 2 * rows * at.pitch
             check(at.all_tiles(at.weight, *ap, p, back, back + 4 * rows, *yp, te, tl, max_mtiles, epilogue, at.status, at.sms, stream_ptr()),
                   "grouped_gemm_w4")
