@@ -310,6 +310,7 @@ w4_rows_kernel(const W4Weight w, const bf16* x, int ldx, bf16* C, int ldc, const
     // a wait that runs out leaves numbers that are wrong and an error for the host
     if (!mbar_wait(bar, 0, status, PIE_ERR_WAIT_TMA)) drain(bar, 0);
     if (KIND == W4_FP4) w4_batch_fp16(batch, row_bytes, M, have >> 3, tops);
+    __syncwarp();                                       // lanes may leave the wait one by one; an MMA is all of theirs
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -370,6 +371,7 @@ w4_rows_kernel(const W4Weight w, const bf16* x, int ldx, bf16* C, int ldc, const
             const float4 v = here(r, col);
             st_cluster_v4(map_to_cta(far_at + ((col << mine_shift) + (r & (mine - 1))) * 4, r >> mine_shift), v.x, v.y, v.z, v.w);
         }
+        __syncwarp();                                   // some lanes have a turn more
         cluster_sync_all();
     }
     const bool glu = epi == EPI_SWIGLU || epi == EPI_GEGLU;
@@ -578,6 +580,7 @@ w4_experts_kernel(const W4Weight w, const bf16* x, int ldx, bf16* C, int ldc, co
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[0][j] = 0.f;
         xr[0] = x0;
+        __syncwarp();                              // lanes leave the wait and the last step's stores one by one; an MMA is all of theirs
     };
     auto leave = [&]() {                           // false where a wait ran out
         if (KIND == W4_FP4) w4_unscale(acc[0], top + 2 * t);
@@ -1072,6 +1075,7 @@ w4_tile_kernel(const __grid_constant__ W4Maps maps, const W4Weight w, const floa
             for (int g = odd; g * 16 < t.rows; g += 2) {
                 uint32_t r[16];
                 float v[16];
+                __syncwarp();                // features past the last store nothing
                 tmem_ld_32x16(t_row + g * 16, r);
                 tmem_ld_wait();
 #pragma unroll

@@ -7,6 +7,8 @@ import torch
 from pie_b200 import ops
 from pie_b200.ops import w4
 
+from test_w4_ops import FORMS, close, expert_case, product_case
+
 
 class Rows:
     """bf16 rows as a call on a GPU looks at them, in host memory, that remember the scratch made of them."""
@@ -54,3 +56,28 @@ def test_scratch_lives_until_the_launches_are_made(monkeypatch, most):
     one._gpu = at = Launchers(one, x, most)
     ops.gemm_w4(x, one)
     assert at.alive == ([[True]] if most else [[True, True]])          # the output is made of the rows too
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [FORMS[0], FORMS[2], FORMS[5]], ids=["int4", "int4z", "fp4"])
+def test_lanes_that_part_ahead_of_instructions_of_whole_warps(form):
+    """Batches of which a part of a warp has a turn more before a cluster joins, features past the last inside a warp between reads of
+    tensor memory, experts' steps that few lanes store: right, and the same every time."""
+    for m, n, k in ((1, 64, 16384), (3, 64, 16384), (1, 4096, 14336), (7, 264, 8192), (40, 40, 128), (200, 24, 128), (130, 1000, 256)):
+        k = k // form[3] * form[3]
+        x, w, _, want, room = product_case(m, n, k, form)
+        first = ops.gemm_w4(x, w)
+        close(first, want, room)
+        for _ in range(20):
+            assert torch.equal(ops.gemm_w4(x, w), first)
+    for counts in ([1, 0, 3], [2] * 40, [300, 9, 40]):
+        for n, k in ((8, 128), (40, 1024)):
+            a, w, buf, mt, want, room, used = expert_case(counts, n, k, form, ops.EPI_STORE)
+            for rows in (1, 1 << 40):
+                out = torch.full(want.shape, 3.0, device="cuda").bfloat16()
+                ops.grouped_gemm(a, w, buf.tile_expert, out, mt, ops.EPI_STORE, buf.tile_list, rows)
+                close(out, want, room)
+                again = torch.full(want.shape, 3.0, device="cuda").bfloat16()
+                ops.grouped_gemm(a, w, buf.tile_expert, again, mt, ops.EPI_STORE, buf.tile_list, rows)
+                assert torch.equal(again, out)
+    ops.check_kernel_status()
