@@ -151,7 +151,7 @@ def _build_drivers_direct(m: ModelSection):
         if m.path:
             _, w = loader.load_checkpoint(m.path, "cpu", dtype="float32")
             cfg.dtype = "float32"
-        return [TorchDriver(cfg, "cpu", weights=w, num_pages=4096, page_size=d.kv_page_size,
+        return [TorchDriver(cfg, "cpu", weights=w, num_pages=4096, page_size=d.kv_page_size, weight_dtype=d.weight_dtype,
                             vision=_vision_encoder(m, cfg, "cpu", torch.float32),
                             audio=_audio_encoder(m, cfg, "cpu", torch.float32))], cfg, tok, comm
     groups = calculate_topology(d.device, d.tensor_parallel_size)

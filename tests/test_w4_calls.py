@@ -81,3 +81,15 @@ def test_lanes_that_part_ahead_of_instructions_of_whole_warps(form):
                 ops.grouped_gemm(a, w, buf.tile_expert, again, mt, ops.EPI_STORE, buf.tile_list, rows)
                 assert torch.equal(again, out)
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("preset", ["tiny-llama", "tiny-qwen3-moe"])
+def test_the_cpu_driver_that_a_configuration_makes_has_its_weights_in_4_bits(preset):
+    from pie_b200.server import config as cfgmod
+    from pie_b200.server.serve import _build_drivers_direct
+    text = f'[[model]]\nname = "m"\npreset = "{preset}"\n[model.driver]\ntype = "cpu"\n'
+    held = []
+    for key in ("", 'weight_dtype = "int4"\n'):
+        (drv,), _, _, _ = _build_drivers_direct(cfgmod.parse(text + key).model[0])
+        held.append([isinstance(lw["wqkv"], ops.W4Linear) for lw in drv.model.w["layers"]])
+    assert not any(held[0]) and all(held[1])
