@@ -344,7 +344,7 @@ def quantize_layers(w: dict, cfg: ModelConfig, weight_dtype: str) -> dict:
     for lw in w["layers"]:
         for key, rows in ({**_LINEARS, **_EXPERTS} if weight_dtype == "int4" else _EXPERTS).items():
             t = lw.get(key)
-            if not torch.is_tensor(t) or t.dtype not in (torch.bfloat16, torch.float32) or t.shape[-2] % rows or t.shape[-1] % 32:
+            if not torch.is_tensor(t) or t.dtype not in (torch.bfloat16, torch.float16, torch.float32) or t.shape[-2] % rows or t.shape[-1] % 32:
                 continue
             if weight_dtype == "mxfp4":
                 lw[key] = quantize_w4(t, 32, kind="fp4")

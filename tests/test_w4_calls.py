@@ -93,3 +93,11 @@ def test_the_cpu_driver_that_a_configuration_makes_has_its_weights_in_4_bits(pre
         (drv,), _, _, _ = _build_drivers_direct(cfgmod.parse(text + key).model[0])
         held.append([isinstance(lw["wqkv"], ops.W4Linear) for lw in drv.model.w["layers"]])
     assert not any(held[0]) and all(held[1])
+
+
+def test_layers_in_fp16_are_quantised():
+    from pie_b200.models.config import preset
+    from pie_b200.models.weights import quantize_layers, random_weights
+    cfg = preset("tiny-llama")
+    for lw in quantize_layers(random_weights(cfg, "cpu", torch.float16), cfg, "int4")["layers"]:
+        assert isinstance(lw["wqkv"], ops.W4Linear) and isinstance(lw["wo"], ops.W4Linear)
