@@ -127,7 +127,8 @@ class W4Linear:
         q._hold(packed, scale, zero, factor, tuple(shape), group, kind)
         return q
 
-    def _hold(self, packed, scale, zero, factor, shape, group, kind):
+    def _hold(self, packed, scale, zero, factor, shape, group, kind, written: bool = False):
+        """`written`: what wrote the tensors is done."""
         self.packed, self.scale, self.zero, self.factor = packed, scale, zero, factor
         self.shape, self.group, self.kind = torch.Size(shape), group, kind
         e = shape[0] if self.dims == 3 else 1
@@ -136,7 +137,8 @@ class W4Linear:
         self._gpu = None
         if packed.is_cuda:
             # the products request weights before the kernel ahead of them in the stream is done
-            torch.cuda.synchronize(packed.device)
+            if not written:
+                torch.cuda.synchronize(packed.device)
             self._gpu = _OnGpu(self)
 
     @property
@@ -191,11 +193,13 @@ class W4Experts(W4Linear):
         return True
 
     def __getitem__(self, e: int) -> W4Linear:
-        """Expert e's weight, in the same memory."""
+        """Expert e's weight, in the same memory: no wait, and usable while a graph is captured."""
         if not -self.shape[0] <= e < self.shape[0]:
             raise IndexError(f"expert {e} of {self.shape[0]}")
         part = lambda t: t[e % self.shape[0]][None] if t is not None else None
-        return W4Linear.from_packed(part(self.packed), part(self.scale), part(self.zero), part(self.factor), self.shape[1:], self.group, self.kind)
+        q = W4Linear.__new__(W4Linear)
+        q._hold(part(self.packed), part(self.scale), part(self.zero), part(self.factor), self.shape[1:], self.group, self.kind, written=True)
+        return q
 
 
 def quantize_w4(w: torch.Tensor, group: int = 128, kind: str = "int4", asymmetric: bool = False, scale_dtype=torch.bfloat16):

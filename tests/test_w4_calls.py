@@ -7,7 +7,7 @@ import torch
 from pie_b200 import ops
 from pie_b200.ops import w4
 
-from test_w4_ops import FORMS, close, expert_case, product_case
+from test_w4_ops import FORMS, close, expected, expert_case, product_case
 
 
 class Rows:
@@ -101,3 +101,23 @@ def test_layers_in_fp16_are_quantised():
     cfg = preset("tiny-llama")
     for lw in quantize_layers(random_weights(cfg, "cpu", torch.float16), cfg, "int4")["layers"]:
         assert isinstance(lw["wqkv"], ops.W4Linear) and isinstance(lw["wo"], ops.W4Linear)
+
+
+@pytest.mark.gpu
+def test_an_expert_alone_is_taken_without_waiting_and_in_a_graph(monkeypatch):
+    gen = torch.Generator("cuda").manual_seed(2)
+    q = ops.quantize_w4(torch.randn(3, 64, 256, generator=gen, device="cuda"), 64, asymmetric=True)
+    x = torch.randn(5, 256, generator=gen, device="cuda").bfloat16()
+    want, room = expected(x, q[1].dequant(torch.float64))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.gemm_w4(x, q[1])
+    g.replay()
+    close(y, want, room)
+
+    def stop(device=None):
+        raise AssertionError("the device is waited for")
+    monkeypatch.setattr(torch.cuda, "synchronize", stop)
+    assert torch.equal(ops.gemm_w4(x, q[-2]), y)
+    with pytest.raises(AssertionError):                                # a weight of its own does wait for what wrote it
+        ops.W4Linear.from_packed(q.packed[:1], q.scale[:1], q.zero[:1], q.factor[:1], (64, 256), 64, "int4")
