@@ -550,6 +550,14 @@ def gemm_fp8w(x, q: "Fp8Linear", residual=None, epilogue: int = EPI_STORE, mode:
             raise ValueError(f"gemm_fp8w: 8-bit rows come with dense fp32 scales [M, {q.scale.shape[1]}]")
         if x.is_cuda and (q.shape[1] % 16 or q.shape[0] % 16 or mode == "dequant"):
             raise ValueError("gemm_fp8w: 8-bit rows need the fused kernel, and weights whose sides are multiples of 16")
+        if epilogue not in (EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU) or (residual is not None) != (epilogue == EPI_RESIDUAL):
+            raise ValueError("gemm_fp8w: 8-bit rows go with EPI_STORE, EPI_SWIGLU and EPI_RESIDUAL, and a residual with the last alone")
+        if any(t.device != x.device for t in (q, residual) if t is not None):
+            raise ValueError("gemm_fp8w: rows, weight and residual must be on one device")
+        if residual is not None and (tuple(residual.shape) != (x.shape[0], q.shape[0]) or (x.is_cuda and residual.dtype != torch.bfloat16)):
+            raise ValueError(f"gemm_fp8w: residual {residual.dtype} {tuple(residual.shape)} for outputs of {x.shape[0]} x {q.shape[0]}")
+        if residual is not None and x.is_cuda and (_dense16(residual, residual.shape) is None or residual.stride(0) >= 2 ** 31):
+            residual = residual.clone(memory_format=torch.contiguous_format)
         if not x.is_cuda:
             x = (x.float() * sx.repeat_interleave(FP8_BLOCK, dim=1)[:, :q.shape[1]]).to(residual.dtype if residual is not None else torch.float32)
     if not x.is_cuda:
