@@ -138,7 +138,7 @@ class Transformer:
         """RMS norm of the stream for the product with `w`: bf16 rows, or, where `fp8_norm` is on and `w` is a block-scaled fp8 weight whose
         fused kernel such a batch takes, rows in 8 bits straight from the norm. `reuse`: something else reads the rows, too."""
         if self.fp8_norm and not reuse and isinstance(w, ops.Fp8Linear) and self.gemm_backend == "tcgen05" and h.is_cuda:
-            if h.dtype == torch.bfloat16 and ops.fp8_takes_rows8(h.shape[0], w):
+            if h.dtype == torch.bfloat16 and h.shape[1] <= ops.NORM_FP8_COLS and ops.fp8_takes_rows8(h.shape[0], w):
                 return ops.rmsnorm_fp8(h, w_norm, self.cfg.rms_norm_eps)
         return ops.rmsnorm(h, w_norm, self.cfg.rms_norm_eps)
 

@@ -423,6 +423,7 @@ def quant_act_fp8(x: torch.Tensor):
 
 
 _NORM_FP8 = {}         # per device
+NORM_FP8_COLS = 16384  # most columns of a row: a block holds one in registers
 
 
 def _dense16(t, shape):
@@ -445,7 +446,7 @@ def _shifted(dst, rows, m: int, k: int) -> bool:
 def _norm_fp8(name, x, delta, w, eps, w_offset, residual_out):
     k = w.shape[0] if w.dim() == 1 else 0
     # the common call, checked in one go: the kernel takes less time than a careful look at its arguments
-    if x.is_cuda and x.dim() == 2 and 0 < k <= 16384 and not k & 15 and w.dtype is torch.bfloat16 and w.is_contiguous() and not w.data_ptr() & 15:
+    if x.is_cuda and x.dim() == 2 and 0 < k <= NORM_FP8_COLS and not k & 15 and w.dtype is torch.bfloat16 and w.is_contiguous() and not w.data_ptr() & 15:
         dev, m = x.get_device(), x.shape[0]
         shape = (m, k)
         xa = _dense16(x, shape)
@@ -483,8 +484,8 @@ def _norm_fp8_any(name, x, delta, w, eps, w_offset, residual_out):
         return reference.rmsnorm_fp8(x, w, eps, w_offset)
     if any(t is not None and t.dtype != torch.bfloat16 for t in (x, delta, w)):
         raise ValueError(f"{name}: rows and weight are bf16 on the GPU")
-    if k % 16 or not 0 < k <= 16384:
-        raise ValueError(f"{name}: rows of {k} columns (multiples of 16 up to 16384)")
+    if k % 16 or not 0 < k <= NORM_FP8_COLS:
+        raise ValueError(f"{name}: rows of {k} columns (multiples of 16 up to {NORM_FP8_COLS})")
     if m == 0:
         return x.new_empty((0, k), dtype=torch.float8_e4m3fn), x.new_empty((0, (k + FP8_BLOCK - 1) // FP8_BLOCK), dtype=torch.float32)
     with torch.cuda.device(x.device):

@@ -48,3 +48,19 @@ def test_refused_on_the_gpu_and_residuals_of_any_layout(m, n, k):
         close(ops.gemm_fp8w(rows, q, residual=at, epilogue=ops.EPI_RESIDUAL), want, room)
     assert ops.gemm_fp8w((rows[0][:0], rows[1][:0]), q).shape == (0, n)
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("k,rows8", [(4096, True), (16384, True), (16400, False)])
+def test_norms_of_rows_that_are_too_long_for_8_bits_stay_in_bf16(monkeypatch, k, rows8):
+    """A model's choice between its two norms, by the sizes that each of them takes."""
+    from types import SimpleNamespace
+
+    from pie_b200.models.transformer import Transformer
+    said = []
+    monkeypatch.setattr(ops, "rmsnorm_fp8", lambda h, w, eps: said.append(8))
+    monkeypatch.setattr(ops, "rmsnorm", lambda h, w, eps: said.append(16))
+    model = SimpleNamespace(fp8_norm=True, gemm_backend="tcgen05", cfg=SimpleNamespace(rms_norm_eps=1e-6))
+    h = SimpleNamespace(is_cuda=True, dtype=torch.bfloat16, shape=(5, k))
+    q = ops.Fp8Linear(torch.zeros(16, k).to(torch.float8_e4m3fn), torch.ones(16, -(-k // 128)))
+    Transformer._norm_rows(model, h, None, q)
+    assert said == [8 if rows8 else 16]
