@@ -446,7 +446,8 @@ def _shifted(dst, rows, m: int, k: int) -> bool:
 def _norm_fp8(name, x, delta, w, eps, w_offset, residual_out):
     k = w.shape[0] if w.dim() == 1 else 0
     # the common call, checked in one go: the kernel takes less time than a careful look at its arguments
-    if x.is_cuda and x.dim() == 2 and 0 < k <= NORM_FP8_COLS and not k & 15 and w.dtype is torch.bfloat16 and w.is_contiguous() and not w.data_ptr() & 15:
+    if x.is_cuda and x.dim() == 2 and 0 < k <= NORM_FP8_COLS and not k & 15 and w.dtype is torch.bfloat16 and w.is_contiguous() \
+            and not w.data_ptr() & 15:
         dev, m = x.get_device(), x.shape[0]
         shape = (m, k)
         xa = _dense16(x, shape)
@@ -649,7 +650,8 @@ def grouped_gemm(a, w, tile_expert, out, max_mtiles: int, epilogue: int = EPI_ST
                  rows_in_use: Optional[int] = None):
     """out[tile rows] = a[tile rows] @ w[tile_expert[tile]].T for every used 128-row tile. w [E,N,K]. `tile_list` (as `moe_align`
     writes it) limits the work to the rows in use; other rows of `out` are left alone. w may be a `W4Experts`; its kernel is chosen by
-    the number of `rows_in_use` (at most; the device alone has the exact one), any gives the same product."""
+    the number of `rows_in_use` (at most; the device alone has the exact one), any gives the same product up to rounding. Without it the tiles' room
+    counts, 128 rows or more: callers of a few rows should say so (1 token of 2 of 8 experts of 4096 x 4096: 9.1 us, 19.8 without)."""
     if isinstance(w, W4Experts):
         return grouped_gemm_w4(a, w, tile_expert, out, max_mtiles, epilogue, tile_list, rows_in_use)
     e, n, k = w.shape

@@ -34,10 +34,10 @@ def differences(rows, k, gen):
 
 
 def assert_differences(y, x, w64, rounded):
-    """Few rows: codes and scales are exact, and so is everything for one scale in bf16 times q - 8 (4 + 8 bits, of which the kernel's fp16 holds
-    11: |q - 8| is 8 or has three), and for e2m1 times a power of two. Others (`rounded`) are rounded once to fp16, by 2^-11 of the weight at
-    most. The sum is of two products: some roundings of 2^-22 of the larger. The output is rounded to bf16 (2^-8). A weight rounded to bf16 would be off by
-    up to 2^-8 of it, which is more than all of this for most differences of neighbouring codes."""
+    """Few rows: codes and scales are exact, and so is everything for one scale in bf16 times q - 8 (4 + 8 bits, of which the kernel's fp16
+    holds 11: |q - 8| is 8 or has three), and for e2m1 times a power of two. Others (`rounded`) are rounded once to fp16, by 2^-11 of the
+    weight at most. The sum is of two products: some roundings of 2^-22 of the larger. The output is rounded to bf16 (2^-8). A weight rounded
+    to bf16 would be off by up to 2^-8 of it, which is more than all of this for most differences of neighbouring codes."""
     want, size = x.double() @ w64.T, x.double().abs() @ w64.abs().T
     room = size * ((2.0 ** -11 if rounded else 0.0) + 2.0 ** -20)
     off = (y.double() - want).abs() - (room + 2.0 ** -8 * (want.abs() + room))
