@@ -7,8 +7,8 @@
 // (nibbles 0, 4, 1, 5; e2m1: 0, 1, 2, 3) and g + 8 (nibbles 2, 6, 3, 7; e2m1: 4, 5, 6, 7). A load of a tile is so one 16-byte load
 // per lane, all of it used. Scales and zero points lie as [128 rows][group][row tile][8] pairs (row g, row g + 8). Scales are fp16,
 // multiplied by a power of two per row that brings the row's largest to [2^14, 2^15), or for e2m1 [2^10, 2^11); `factor` undoes it.
-// bf16 and fp16 scales are so held exactly down to 2^-24 of the row's largest, and to 2^-35 of it below. Rows are padded to 128,
-// columns to 64, with codes of value zero and scales of zero.
+// bf16 and fp16 scales are so held exactly down to 2^-24 of the row's largest; smaller ones lose bits, and below 2^-39 of it (e2m1: 2^-35) they
+// are zero. Rows are padded to 128, columns to 64, with codes of value zero and scales of zero.
 //
 // Counterpart of the reference's W4A16 products (driver/cuda/src/kernels/dequant_wna16.cu and its mma.sync GEMM).
 #include <atomic>
@@ -636,17 +636,18 @@ w4_experts_kernel(const W4Weight w, const bf16* x, int ldx, bf16* C, int ldc, co
 // registers; up to 128 rows of the batch are its columns, brought by TMA. Shared memory so holds the weights' codes only, and a weight is
 // expanded once per 128 rows of the batch (256 leave an SM one CTA: no faster for one weight, 5 to 30 % slower over experts).
 //
-// Why fp16: an integer of -8 .. 7 times a bf16 scale fits its 11 bits, others (zero points, fp16 scales) are off by 2^-12, where bf16 operands would
-// round each weight by 2^-8. The batch's rows go there by w4_rows_fp16_kernel, each times a power of two that brings its largest value to
-// [2^14, 2^15): a bf16 value keeps all its bits down to 2^-29 of the row's largest.
+// Why fp16: an integer of -8 .. 7 times a bf16 scale fits its 11 bits, others (zero points, fp16 scales) are off by 2^-11 of the weight at most,
+// where bf16 operands would round each weight by 2^-8. The batch's rows go there by w4_rows_fp16_kernel, each times a power of two that brings
+// its largest value to [2^14, 2^15): a bf16 value keeps all its bits down to 2^-29 of the row's largest.
 //
 // K is split over the CTAs of a cluster where there are few tiles, as in gemm_skinny.cu; partial tiles meet in distributed shared memory
 // in CTA order. Every mbarrier wait is bounded.
 //
 // Bound by the MMA issuer's way through two blocks: 690 cycles at 48 columns (clocks read in the kernel: its two waits 185 although what they
 // wait for is there, eight MMAs 230, two commits and the loop the rest), 900 at 128, where the MMAs themselves are 192 and 512 by the rate and
-// the expansion of their weights 600; two CTAs of an SM hide a part of that from each other. 2048 rows through 28672 x 4096: 394 us, 74 % of
-// cuBLAS' rate; 48 rows through 6144 x 4096 11.4 us with the conversion, 4096 x 14336 19, 28672 x 4096 23.
+// the expansion of their weights 600; two CTAs of an SM hide a part of that from each other. 2048 rows through 28672 x 4096: 391 us in a
+// graph, 74 % of the rate of a library product of bf16 measured in bursts (calls one after another run into the power limit: 459 us); 48 rows through
+// 6144 x 4096 11.4 us with the conversion, 4096 x 14336 19, 28672 x 4096 23.
 using namespace sm100;
 
 // Work of a launch, in items of up to tile_rows rows: rows [0, M) of one weight, or the rows of a sorted batch (tiles as in gemm_grouped.cu),
@@ -1231,6 +1232,13 @@ static long w4_at_once(int per_sm, int cluster, int num_sms) { return (long)per_
 // with two of each of four.
 // Shares go to warps first; to CTAs where a CTA's part of the batch would outweigh its weights (every CTA of a tile reads all of its share
 // of the batch) or not fit beside a neighbour's. Joining a cluster costs some 0.7 us, so small batches' short rows stay in a CTA.
+// The first: several warps to a tile are fewer tiles to a CTA, and the batch is read that much more often. Measured (us, warps to a tile x CTAs):
+// 10240 x 5120 at 4 rows 4 x 1 9.2, 8 x 1 10.3, 1 x 4 8.9, at 8 rows 2 x 2 9.8, 8 x 1 14.2, 1 x 4 9.4, at 16 rows 1 x 4 12.7, 2 x 4 14.7, 8 x 1
+// 25.1; 4096 x 4096 at 16 rows 2 x 4 5.2, 1 x 8 6.0, 8 x 1 7.6; below 48 KB 6144 x 4096 at 4 rows 8 x 1 5.0, 2 x 4 5.3. The second, 56 KB (72
+// from 17 rows on) of the batch in a CTA: 4096 x 14336 at 16 rows 56 KB 11.5, 112 KB 14.0; 27648 x 5120 at 8 rows 41 KB 17.2, 82 KB 19.5, but
+// 28672 x 4096 at 8 33 KB 17.1, 66 KB 15.9; 14336 x 4096 at 32 rows 66 KB 23.0, 132 KB 27.1. Over seven weights at 2 to 32 rows, int4 and e2m1,
+// the rule is within a tenth of the best in four cases of five; farthest are 28672 x 4096 at 6 rows of e2m1 (22.7, 1 x 1 17.8), 14336 x 4096 at 4
+// of those (12.6, 1 x 2 10.0) and 4096 x 4096 at 32 rows (9.2, 2 x 4 7.5).
 static void w4_rows_split(const W4Weight& w, int M, int unit, int num_sms, int& wk, int& ct) {
     const int blocks = w.blocks(), units = blocks / unit, tiles = w.row_tiles(), enough = M > 16 ? 150 : 256;
     int p = 0;                                          // log2 of all shares
@@ -1294,11 +1302,11 @@ static cudaError_t launch_w4_rows_group(const W4Weight& w, const W4Call& c) {
     return w.group == 32 ? launch_w4_rows_nt<KIND, 32>(w, c) : w.group == 64 ? launch_w4_rows_nt<KIND, 64>(w, c) : launch_w4_rows_nt<KIND, 128>(w, c);
 }
 
-// CTAs that share the K of 128 weight rows in the tensor cores' way: the least of the blocks of 64 columns of a CTA and what the join costs
-// in blocks, where two CTAs of an SM hold each other up by a third. Measured (us, at 48 rows): 4096 x 14336 51 (1), 32 (2), 19 (4); 10240 x 5120
-// 17.0 (2), 15.0 (3); 6144 x 4096 12.8 (2), 20.7 (3, an SM each: two rounds), 11.5 (4); 5120 x 5120 12.5 (3), 12.2 (4); 1024 x 8192 12.5 (4),
-// 10.1 (8); 2048 x 8192 12.5 (4), 18.9 (8: two rounds); 14336 x 1024 8.1 (1), 9.1 (2); 4096 x 1024 7.3 (2), 7.2 (4), of 256 rows 10.9 (2), 12.5
-// (4).
+// CTAs that share the K of 128 weight rows in the tensor cores' way: the least of the blocks of 64 columns of a CTA and what the join costs in
+// blocks, where two CTAs of an SM hold each other up by a third. Measured (us, at 48 rows): 4096 x 14336 45 (1), 28 (2), 21.8 (3), 19.7 (4), 18.4
+// (8); 10240 x 5120 19.9 (1), 16.8 (2), 15.1 (3), 22.2 (4: two rounds); 6144 x 4096 12.5 (2), 12.8 (3), 11.4 (4); 5120 x 5120 13.9 (2), 12.5 (3),
+// 12.3 (4); 1024 x 8192 12.4 (4), 10.1 (8); 2048 x 8192 12.5 (4), 18.9 (8: two rounds); 14336 x 1024 8.1 (1), 9.1 (2); 4096 x 1024 7.3 (2), 7.2
+// (4), of 256 rows 10.9 (2), 12.5 (4). The join of three is set at what leaves them the weights with which four take two rounds.
 static int w4_tile_splits(long items, int blocks, int num_sms) {
     int best = 1;
     double least = 0;
@@ -1407,7 +1415,9 @@ static int w4_tiles(const W4Weight& w, const W4Call& c, const W4Rows16& r, const
     W4Work work{(int4*)items_at, c.M, 0};
     int rows_per_tile = 0;                  // blocks of the conversion per 128 rows of a sorted batch
     if (sorted) {
-        // as wide as the experts' rows are on average, at most (the counts are on the device): an expert with more rows takes several items
+        // About as wide as the experts' rows are on average (the counts are on the device): an expert with more rows takes several items.
+        // Measured (us, items of 32 / 64 / 128 rows): 4 of 32 experts of 5760 x 2880, 8 rows each 71 / 71 / 80, 16 82 / 75 / 84, 24 85 / 79 / 86,
+        // 32 105 / 87 / 89, 50 130 / 95 / 97; 8 of 128 of 1536 x 2048, 8 rows 58 / 59 / 65, 16 71 / 71 / 75, 25 86 / 75 / 80, 38 104 / 90 / 93.
         const long least = tiles.max_mtiles > w.experts ? (tiles.max_mtiles - w.experts) * (long)GEMM_BM / w.experts : 0;
         work.tile_rows = least <= 8 ? 32 : least <= 24 ? 64 : 128;
         // Some 2500 blocks (us, with 16 / 32 / 64 / 128 per tile: 1500 tokens of 4 of 32 experts 217 / 210 / 209 / 208, 512 of 2 of 8 80 / 69 / 64

@@ -54,8 +54,9 @@ class _OnGpu:
 
 class W4Linear:
     """Weight [N, K] in 4-bit codes. `codes` [N, K] uint8 (0..15), `scale` [N, K / group] bf16 or fp16, `zero` [N, K / group] uint8 (0..15,
-    "int4" only; 8 without it), group = 32, 64 or 128. The tensors it holds are not to be changed: products read them while the kernel ahead
-    of them in the stream is still running."""
+    "int4" only; 8 without it), group = 32, 64 or 128. A scale is held exactly down to 2^-24 of its row's largest, with fewer bits below, and as zero
+    below 2^-39 of it (e2m1: 2^-35). The tensors it holds are not to be changed: products read them while the kernel ahead of them in the
+    stream is still running."""
 
     dims = 2
 
