@@ -121,3 +121,86 @@ def test_an_expert_alone_is_taken_without_waiting_and_in_a_graph(monkeypatch):
     assert torch.equal(ops.gemm_w4(x, q[-2]), y)
     with pytest.raises(AssertionError):                                # a weight of its own does wait for what wrote it
         ops.W4Linear.from_packed(q.packed[:1], q.scale[:1], q.zero[:1], q.factor[:1], (64, 256), 64, "int4")
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits():
+    """Batches of more than 2^31 elements: their first and last rows' products, norms and experts' products."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    m, n, k = 270000, 64, 8192
+    q = ops.quantize_w4(torch.randn(n, k, generator=gen, device="cuda"), 128)
+    x = torch.randn(512, k, generator=gen, device="cuda").bfloat16().repeat(528, 1)[:m]
+    assert x.numel() > 2 ** 31
+    ends = torch.tensor([0, 1, 511, m - 70, m - 1], device="cuda")
+    y = ops.gemm_w4(x, q)
+    close(y[ends], *expected(x[ends], q.dequant(torch.float64)))
+    assert torch.equal(y[:512], y[512 * 400:512 * 401])                # the same rows in other places
+    w = torch.ones(k, device="cuda").bfloat16()
+    x8, sx = ops.rmsnorm_fp8(x, w, 1e-6)
+    want8, want = ops.rmsnorm_fp8(x[ends].clone(), w, 1e-6)
+    assert torch.equal(sx[ends], want) and torch.equal(x8[ends].view(torch.uint8), want8.view(torch.uint8))
+    e, mt = 2, m // 128
+    twice = lambda t: torch.cat([t, t]) if t is not None else None
+    experts = ops.W4Experts.from_packed(twice(q.packed), twice(q.scale), twice(q.zero), twice(q.factor), (e, n, k), 128, "int4")
+    buf = ops.MoeBuffers(m, 8, 8, e, 1, "cuda")
+    for counts in ([m // 256 * 128, 100], [3, (mt - 2) * 128 + 5]):
+        buf.counts.copy_(torch.tensor(counts, dtype=torch.int32))
+        ops.moe_align(buf, mt)
+        first = -(-counts[0] // 128) * 128                             # the second expert's first row
+        at = torch.tensor([0, counts[0] - 1, first, first + counts[1] - 1], device="cuda")
+        for rows in (1, 1 << 40):
+            out = torch.zeros(mt * 128, n, device="cuda").bfloat16()
+            ops.grouped_gemm(x, experts, buf.tile_expert, out, mt, ops.EPI_STORE, buf.tile_list, rows)
+            close(out[at], *expected(x[at], q.dequant(torch.float64)))
+            assert not out[first + counts[1]:].any() and not out[counts[0]:first].any()
+    ops.check_kernel_status()
+
+
+@pytest.mark.gpu
+def test_calls_of_several_threads():
+    """Threads that share weights, each on a stream of its own and all on one: every result is what the call alone gives."""
+    import threading
+    cases = [product_case(m, 512, 2048, FORMS[i]) for m, i in ((1, 0), (5, 2), (40, 5), (300, 3))]
+    mixed = [expert_case([3, 0, 200, 40], 320, 576 // FORMS[i][3] * FORMS[i][3], FORMS[i], ops.EPI_STORE, seed=i) for i in (0, 5)]
+    torch.cuda.synchronize()
+    runs = [lambda c=c: ops.gemm_w4(c[0], c[1]) for c in cases]
+    for c in mixed:
+        for rows in (1, 1 << 40):
+            runs.append(lambda c=c, rows=rows: ops.grouped_gemm(c[0], c[1], c[2].tile_expert, torch.full(c[4].shape, 3.0, device="cuda").bfloat16(),
+                                                                c[3], ops.EPI_STORE, c[2].tile_list, rows))
+    first = [f() for f in runs]
+    torch.cuda.synchronize()
+    for own in (False, True):
+        wrong, shared = [], torch.cuda.Stream()
+
+        def work(i):
+            with torch.cuda.stream(torch.cuda.Stream() if own else shared):
+                for _ in range(30):
+                    y = runs[i]()
+                    if not torch.equal(y, first[i]):
+                        wrong.append(i)
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(len(runs))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not wrong, wrong
+    ops.check_kernel_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 6, 40])
+def test_rows_that_share_memory_or_have_odd_strides(m):
+    x, w, r, want, room = product_case(m, 128, 384, FORMS[0], ops.EPI_RESIDUAL)
+    one = x[:1].expand(m, -1)
+    close(ops.gemm_w4(one, w, r, ops.EPI_RESIDUAL), *expected(one, w.dequant(torch.float64), r, ops.EPI_RESIDUAL))
+    close(ops.gemm_w4(x, w, r[:1].expand(m, -1), ops.EPI_RESIDUAL), *expected(x, w.dequant(torch.float64), r[:1].expand(m, -1), ops.EPI_RESIDUAL))
+    flat = torch.randn(384 + 5 * m, device="cuda").bfloat16()
+    near = flat.as_strided((m, 384), (5, 1))                           # rows that begin five elements after one another
+    close(ops.gemm_w4(near, w), *expected(near, w.dequant(torch.float64)))
+    near = flat.as_strided((m, 384), (8 if m < 6 else 0, 1))
+    close(ops.gemm_w4(near, w), *expected(near, w.dequant(torch.float64)))
+    gain = torch.ones(384, device="cuda").bfloat16()
+    a, b = ops.rmsnorm_fp8(near, gain, 1e-6), ops.rmsnorm_fp8(near.clone(), gain, 1e-6)
+    assert torch.equal(a[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(a[1], b[1])
