@@ -161,7 +161,7 @@ class W4Linear:
         return self.dequant(torch.float32)
 
     def dequant(self, dtype=torch.bfloat16) -> torch.Tensor:
-        """The weight in `dtype`, each value rounded once."""
+        """The weight in `dtype`, each value rounded once. `gemm` over it right away wants `fresh_w=True`, as over any weight just written."""
         if not self.is_cuda or dtype != torch.bfloat16:
             return self._plain(dtype)
         out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
